@@ -9,9 +9,10 @@
  * (NULL: the default stream). Calls only queue kernels: they never
  * synchronize, allocate or copy, so they can be recorded into a HIP graph.
  * Strides are in elements of the row they step over (bytes for 8-bit values
- * and scales, words for masks); the last axis is dense. Calls return TK_OK
- * or one of the TK_E_* codes of toktier_hip.h (the values are repeated
- * below), with a message in tk_head_last_error() (per thread).
+ * and scales, words for masks), and an input of one row may have any; the
+ * last axis is dense. Calls return TK_OK or one of the TK_E_* codes of
+ * toktier_hip.h (the values are repeated below), with a message in
+ * tk_head_last_error() (per thread).
  *
  * 8-bit values are OCP e4m3 ("float8_e4m3fn"). A scale is one byte, e8m0: it
  * stands for 2^(byte - 127), and 255 for NaN. Row r of k values has
@@ -76,9 +77,9 @@ typedef struct tkh_norm {
  * (TKH_BF16 or TKH_F16). The unit adds the products of 8-bit values to each
  * other with about 16 bits to the largest of a group and the groups in 32
  * bits: about 2^-16 of a sum, which 16-bit results do not show and 32-bit
- * ones would, so there are none. Rows of a and
- * w are 16-byte aligned (base and stride) and read in whole 16-byte pieces;
- * what lies beyond k does not count. */
+ * ones would, so there are none. Rows of a and w are 16-byte aligned (base,
+ * and stride where there are several) and read in whole 16-byte pieces; what
+ * lies beyond k does not count. */
 typedef struct tkh_matmul {
     const void* a;          /* [m, k] e4m3 */
     const void* a_scale;    /* [m, ceil(k / 128)] e8m0 */

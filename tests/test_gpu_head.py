@@ -597,3 +597,16 @@ def test_refusals_on_the_device():
         head.sample(x, u[:1])
     with pytest.raises(ValueError, match="on cpu"):
         head.sample(x, u.cpu())
+
+
+@pytest.mark.parametrize("k", [1000, 1111, 4104, 6144])
+def test_matmul_of_a_single_row_of_any_stride(k):
+    """A contiguous row whose length is no multiple of 16, as a and as w."""
+    g = gen(k)
+    one, many = quantized(g, 1, k), quantized(g, 90, k)
+    tight = torch.empty(1, k, dtype=torch.uint8, device="cuda")
+    tight.copy_(one[0].view(torch.uint8))
+    tight = tight.view(torch.float8_e4m3fn)
+    assert tight.stride(0) == k
+    assert torch.equal(head.matmul_fp8(tight, one[1], *many), head.matmul_fp8(*one, *many))
+    assert torch.equal(head.matmul_fp8(*many, tight, one[1]), head.matmul_fp8(*many, *one))

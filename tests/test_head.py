@@ -183,3 +183,63 @@ def test_quantize_edges():
         head.quantize_fp8(torch.zeros(4))
     with pytest.raises(ValueError):
         head.OutputHead(torch.ones(256), q, s, vocab=2)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="a GPU is visible")
+def test_strides_of_a_single_row_are_not_asked_about():
+    """No kernel steps from one row to the next where there is one: refused
+    for the missing device alone."""
+    p = 1 << 20
+    mm = [p, p, p, p, p, 1, 64, 1000, 1000, 8, 1008, 8, 64, 1, 0]
+    assert call("tk_head_matmul", head._MATMUL, *mm) == -3
+    mm = [p, p, p, p, p, 4, 1, 1000, 1008, 8, 1000, 8, 1, 1, 0]
+    assert call("tk_head_matmul", head._MATMUL, *mm) == -3
+    norm = [p, p, p, p, p, p, 1, 256, -8, -8, 256, 2, -8, 1e-6, 0, 0, 0]
+    assert call("tk_head_norm", head._NORM, *norm) == -3
+
+
+class Stand:
+    """What the Python side calls: notes it and queues nothing."""
+
+    def __init__(self):
+        self.calls = []
+
+    def tk_head_norm(self, args, stream):
+        self.calls.append(("norm", head._NORM.unpack(args)))
+        return 0
+
+    def tk_head_matmul(self, args, stream):
+        self.calls.append(("matmul", head._MATMUL.unpack(args)))
+        return 0
+
+    def tk_head_sample(self, args, stream):
+        self.calls.append(("sample", head._SAMPLE.unpack(args)))
+        return 0
+
+    def tk_head_sample_workspace(self, rows, vocab, dtype):
+        return 64
+
+    def names(self):
+        return [name for name, _ in self.calls]
+
+
+class Place:
+    index = 0
+
+
+@pytest.fixture
+def stand(monkeypatch):
+    """The checks of ``toktier_amd.head`` on CPU tensors."""
+    s = Stand()
+    monkeypatch.setattr(head, "_lib", s)
+    monkeypatch.setattr(head, "_raw_stream", lambda device: 0)
+    monkeypatch.setattr(head, "_gpu", lambda t, name: Place)
+    monkeypatch.setattr(head, "_on", lambda t, device, name: None)
+    return s
+
+
+def test_a_weight_of_one_value_is_dense(stand):
+    head.rms_norm_fp8(torch.randn(3, 1), torch.randn(1, 5)[:, 0])
+    assert stand.names() == ["norm"]
+    with pytest.raises(ValueError, match="dense"):
+        head.rms_norm_fp8(torch.randn(3, 2), torch.randn(2, 5)[:, 0])

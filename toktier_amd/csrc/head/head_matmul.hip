@@ -568,7 +568,8 @@ extern "C" int tk_head_matmul(const tkh_matmul* args, void* stream) {
         return fail(TKH_E_UNSUPPORTED, "out dtype %d", p.out_dtype);
     if (p.m == 0 || p.n == 0) return TKH_OK;
     if (!p.a || !p.a_scale || !p.w || !p.w_scale || !p.c) return fail(TKH_E_INVALID_ARG, "a null pointer");
-    if (p.a_stride % 16 || p.w_stride % 16 || (uintptr_t)p.a % 16 || (uintptr_t)p.w % 16)
+    // a single row's stride is stepped over by no kernel
+    if ((p.m > 1 && p.a_stride % 16) || (p.n > 1 && p.w_stride % 16) || (uintptr_t)p.a % 16 || (uintptr_t)p.w % 16)
         return fail(TKH_E_SHAPE, "rows of a and w are 16-byte aligned");
     const int64_t blocks = ceil_div(p.k, kBlock);
     if ((p.m > 1 && (p.a_stride < p.k || p.a_scale_stride < blocks)) ||

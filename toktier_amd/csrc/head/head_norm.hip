@@ -180,8 +180,8 @@ extern "C" int tk_head_norm(const tkh_norm* args, void* stream) {
         return fail(TKH_E_SHAPE, "rows of q are 16-byte aligned and at least %lld long", (long long)padded);
     if (p.scale_stride < padded / kBlock)
         return fail(TKH_E_SHAPE, "scale rows of %lld", (long long)p.scale_stride);
-    if ((p.rows > 1 && p.x_stride < 0) || (p.residual && p.residual_stride < 0) ||
-        (p.residual_out && p.rows > 1 && p.out_stride < p.k))
+    if (p.rows > 1 && (p.x_stride < 0 || (p.residual && p.residual_stride < 0) ||
+                       (p.residual_out && p.out_stride < p.k)))
         return fail(TKH_E_SHAPE, "a row stride");
     DeviceScope scope(p.device);
     if (scope.status() != TKH_OK) return scope.status();

@@ -146,7 +146,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *,
         raise TypeError(f"x is {kind}: float32, bfloat16 or float16 is wanted")
     x2 = _rows(x, "x")
     rows, k = x2.shape
-    if weight.shape != (k,) or weight.stride(0) != 1:
+    if weight.shape != (k,) or (k > 1 and weight.stride(0) != 1):
         raise ValueError(f"weight has shape {tuple(weight.shape)}: ({k},), dense, is wanted")
     weight_kind = weight.dtype
     if weight_kind != kind and weight_kind != torch.float32:
@@ -211,8 +211,8 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor,
     ``a``: ``[..., k]``, ``w``: ``[n, k]`` of float8_e4m3fn, their scales
     ``[..., ceil(k / 128)]`` of float8_e8m0fnu (or its bytes as uint8). Rows
     start at multiples of 16 bytes (``rms_norm_fp8`` and ``quantize_fp8`` give
-    such rows for any k). The result is ``[..., n]``, its rows at a multiple
-    of 16 bytes in memory, or ``out``."""
+    such rows for any k; of a single row only the address counts). The result
+    is ``[..., n]``, its rows at a multiple of 16 bytes in memory, or ``out``."""
     device = _gpu(a, "a")
     dtype = _DTYPES.get(out_dtype if out is None else out.dtype)
     if dtype is None or dtype == TKH_F32:
