@@ -610,3 +610,23 @@ def test_matmul_of_a_single_row_of_any_stride(k):
     assert tight.stride(0) == k
     assert torch.equal(head.matmul_fp8(tight, one[1], *many), head.matmul_fp8(*one, *many))
     assert torch.equal(head.matmul_fp8(*many, tight, one[1]), head.matmul_fp8(*many, *one))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("k", [1, 256, 1000, 5001])
+def test_one_axis_is_one_row(k, dtype):
+    """``[k]`` gives what ``[1, k]`` gives, the sum in place among it."""
+    g = gen(k)
+    x, r = randn(g, k).to(DT[dtype]), randn(g, k).to(DT[dtype])
+    norm_w, w = (1 + 0.2 * randn(g, k)).to(DT[dtype]), quantized(g, 77, k)
+    want = head.rms_norm_fp8(x[None], norm_w, residual=r[None])
+    keep = r.clone()
+    got = head.rms_norm_fp8(x, norm_w, residual=r, residual_out=r)
+    assert got.residual is r and got.q.shape == (k,)
+    for a, b in ((got.q.view(torch.uint8), want.q.view(torch.uint8)),
+                 (got.scale.view(torch.uint8), want.scale.view(torch.uint8)),
+                 (r, want.residual)):
+        assert torch.equal(a, b[0])
+    c = head.matmul_fp8(want.q, want.scale, *w)
+    assert torch.equal(head.matmul_fp8(got.q, got.scale, *w), c[0])
+    assert torch.equal(head.OutputHead(norm_w, *w).logits(x, residual=keep), c[0])

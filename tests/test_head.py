@@ -243,3 +243,35 @@ def test_a_weight_of_one_value_is_dense(stand):
     assert stand.names() == ["norm"]
     with pytest.raises(ValueError, match="dense"):
         head.rms_norm_fp8(torch.randn(3, 2), torch.randn(2, 5)[:, 0])
+
+
+def eight(*shape):
+    return head.quantize_fp8(torch.randn(*shape))
+
+
+@pytest.mark.parametrize("lead", [(), (5,), (2, 3), (0,), (0, 3), (3, 0), (1, 1, 1)])
+@pytest.mark.parametrize("k", [256, 300])
+def test_any_number_of_leading_axes(stand, lead, k):
+    blocks = (k + 127) // 128
+    x, w = torch.randn(*lead, k), torch.ones(k)
+    r = torch.randn(*lead, k)
+    out = head.rms_norm_fp8(x, w, residual=r, residual_out=r)
+    assert out.q.shape == lead + (k,) and out.scale.shape == lead + (blocks,)
+    assert out.residual is r
+    assert head.rms_norm_fp8(x, w, residual=r).residual.shape == x.shape
+    for n in (40, 41):
+        assert head.matmul_fp8(out.q, out.scale, *eight(n, k)).shape == lead + (n,)
+        given = torch.empty(*lead, n, dtype=torch.bfloat16)
+        assert head.matmul_fp8(out.q, out.scale, *eight(n, k), out=given) is given
+        assert head.OutputHead(w, *eight(n, k)).logits(x, residual=r).shape == lead + (n,)
+    # what the kernels are given lies in what comes back
+    args = stand.calls[0][1]
+    assert args[3] == out.q.data_ptr() and args[4] == out.scale.data_ptr() and args[5] == r.data_ptr()
+
+
+def test_next_ids_of_other_than_rows_queues_nothing(stand):
+    out = head.OutputHead(torch.ones(256), *eight(40, 256))
+    for shape in ((256,), (1, 1, 256)):
+        with pytest.raises(ValueError, match="two axes"):
+            out.next_ids(torch.randn(*shape), torch.rand(1))
+    assert stand.names() == []

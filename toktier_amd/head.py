@@ -183,8 +183,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *,
     if padded != k:
         q = q[:, :k]
     if x.dim() != 2:
-        q = q.unflatten(0, x.shape[:-1])
-        scale = scale.unflatten(0, x.shape[:-1])
+        q = q.view(x.shape)
+        scale = scale.view(x.shape[:-1] + (blocks,))
     return NormOutput(q, scale, residual_out)
 
 
@@ -232,7 +232,7 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor,
         c = a.new_empty((m, (n + 7) // 8 * 8), dtype=out_dtype)
         if n % 8:
             c = c[:, :n]
-        out = c if a.dim() == 2 else c.unflatten(0, a.shape[:-1])
+        out = c if a.dim() == 2 else c.view(a.shape[:-1] + (n,))
     else:
         if out.shape != a.shape[:-1] + (n,):
             raise ValueError(f"out has shape {tuple(out.shape)}")
@@ -395,4 +395,6 @@ class OutputHead:
                  residual: torch.Tensor | None = None, **settings) -> Sampled:
         """One token for each of the hidden states ``[rows, k]``; settings as
         in ``sample``."""
+        if x.dim() != 2:
+            raise ValueError("hidden states have two axes")
         return sample(self.logits(x, residual=residual), u, **settings)
