@@ -630,3 +630,26 @@ def test_one_axis_is_one_row(k, dtype):
     c = head.matmul_fp8(want.q, want.scale, *w)
     assert torch.equal(head.matmul_fp8(got.q, got.scale, *w), c[0])
     assert torch.equal(head.OutputHead(norm_w, *w).logits(x, residual=keep), c[0])
+
+
+def test_inputs_that_require_grad_give_the_same_and_no_gradient():
+    g = gen(51)
+    x, r, w = randn(g, 4, 300), randn(g, 4, 300), 1 + 0.2 * randn(g, 300)
+    out = head.OutputHead(w, *head.quantize_fp8(randn(g, 77, 300)))
+    u = torch.rand(4, generator=g, device="cuda")
+    want = head.rms_norm_fp8(x, w, residual=r)
+    ids = out.next_ids(x, u, residual=r)
+    x.requires_grad_(True)
+    got = head.rms_norm_fp8(x, w, residual=r)
+    assert torch.equal(got.q.view(torch.uint8), want.q.view(torch.uint8))
+    assert torch.equal(got.scale.view(torch.uint8), want.scale.view(torch.uint8))
+    assert torch.equal(got.residual, want.residual)
+    with pytest.raises(NotImplementedError, match="rms_norm_fp8"):
+        got.residual.sum().backward()
+    drawn = out.next_ids(x, u, residual=r)
+    assert torch.equal(drawn.ids, ids.ids) and torch.equal(drawn.logprob, ids.logprob)
+    with pytest.raises(NotImplementedError, match="sample"):
+        drawn.logprob.sum().backward()
+    assert x.grad is None
+    with pytest.raises(ValueError, match="residual_out"):
+        head.rms_norm_fp8(x, w, residual=r, residual_out=r)

@@ -275,3 +275,70 @@ def test_next_ids_of_other_than_rows_queues_nothing(stand):
         with pytest.raises(ValueError, match="two axes"):
             out.next_ids(torch.randn(*shape), torch.rand(1))
     assert stand.names() == []
+
+
+def needs(t):
+    return t.requires_grad_(True)
+
+
+def test_outputs_of_inputs_that_require_grad_have_no_backward(stand):
+    x, w, r = torch.randn(2, 256), torch.ones(256), torch.randn(2, 256)
+    plain = head.rms_norm_fp8(x, w, residual=r)
+    assert not any(t.requires_grad for t in plain)
+    for kw in (dict(x=needs(x.clone()), weight=w), dict(x=x, weight=needs(w.clone())),
+               dict(x=x, weight=w, residual=needs(r.clone())),
+               dict(x=needs(x.clone()), weight=w, residual=r)):
+        out = head.rms_norm_fp8(**kw)
+        assert (out.residual is None) == ("residual" not in kw)
+        for t in out:
+            if t is not None:
+                with pytest.raises(NotImplementedError, match="rms_norm_fp8"):
+                    t.float().sum().backward()
+        with torch.no_grad():
+            assert not any(t.requires_grad for t in head.rms_norm_fp8(**kw) if t is not None)
+    # the sum does not depend on the weight
+    out = head.rms_norm_fp8(x, needs(w.clone()), residual=r, residual_out=r)
+    assert out.residual is r and not r.requires_grad and out.q.requires_grad
+
+    a, b = eight(2, 256), eight(40, 256)
+    assert not head.matmul_fp8(*a, *b).requires_grad
+    for n in (40, 41):
+        c = head.matmul_fp8(out.q, out.scale, *eight(n, 256))
+        with pytest.raises(NotImplementedError, match="matmul_fp8"):
+            c.float().sum().backward()
+    logits, u = torch.randn(2, 40), torch.rand(2)
+    t = torch.ones(2)
+    assert not head.sample(logits, u, temperature=t).logprob.requires_grad
+    for kw in (dict(logits=needs(logits.clone())), dict(logits=logits, temperature=needs(t.clone()))):
+        got = head.sample(u=u, **kw)
+        assert not got.ids.requires_grad
+        with pytest.raises(NotImplementedError, match="sample"):
+            got.logprob.sum().backward()
+
+
+def test_nothing_that_requires_grad_is_written_into_a_given_tensor(stand):
+    x, w, r = torch.randn(2, 256), torch.ones(256), torch.randn(2, 256)
+    a, b, out = eight(2, 256), eight(40, 256), torch.empty(2, 40, dtype=torch.bfloat16)
+    grad = needs(r.clone())
+    for kw in (dict(x=needs(x.clone()), weight=w, residual=r, residual_out=r),
+               dict(x=x, weight=w, residual=grad, residual_out=torch.empty_like(r)),
+               dict(x=x, weight=w, residual=r, residual_out=grad)):
+        with pytest.raises(ValueError, match="residual_out"):
+            head.rms_norm_fp8(**kw)
+    with pytest.raises(ValueError, match="out"):
+        head.matmul_fp8(needs(a[0].clone()), a[1], *b, out=out)
+    with pytest.raises(ValueError, match="out"):
+        head.matmul_fp8(*a, *b, out=needs(out.clone()))
+    assert stand.names() == []
+    with torch.no_grad():
+        assert head.rms_norm_fp8(x, w, residual=grad, residual_out=grad).residual is grad
+
+
+def test_an_output_head_holds_its_weights_detached(stand):
+    w = torch.nn.Parameter(torch.ones(256))
+    out = head.OutputHead(w, *head.quantize_fp8(torch.nn.Parameter(torch.randn(40, 256))))
+    assert out.norm_weight.data_ptr() == w.data_ptr()
+    assert not out.logits(torch.randn(2, 256)).requires_grad
+    got = out.next_ids(needs(torch.randn(2, 256)), torch.rand(2))
+    with pytest.raises(NotImplementedError):
+        got.logprob.sum().backward()

@@ -13,7 +13,10 @@ Inputs and outputs are torch tensors on one GPU. Calls queue on torch's
 current stream of that device, never synchronize and can be captured into a
 graph. There is no CPU fallback: a refused call raises ``EngineError`` with
 the library's status and message, a tensor that does not fit raises
-``ValueError`` or ``TypeError`` before anything is queued.
+``ValueError`` or ``TypeError`` before anything is queued. There is no
+backward pass: where an input requires grad so do the outputs, and a backward
+pass that reaches them raises; what would have to be written into ``out`` or
+``residual_out`` is refused there.
 
     head = OutputHead(norm_weight, *quantize_fp8(lm_head))
     out = head.next_ids(hidden, u, residual=residual, temperature=0.7, top_p=0.9)
@@ -120,6 +123,36 @@ def _gpu(t: torch.Tensor, name: str) -> torch.device:
     return device
 
 
+class _NoBackward(torch.autograd.Function):
+    """A call's outputs, as they are, where an input of it requires grad: a
+    backward pass that reaches them raises instead of passing them over."""
+
+    @staticmethod
+    def forward(ctx, call, outputs, *inputs):
+        ctx.call = call
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*[t for t in outputs if not t.is_floating_point()])
+        return outputs
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError(f"{ctx.call} has no backward pass")
+
+
+def _untracked(call: str, outputs: tuple, *inputs) -> tuple:
+    """``outputs`` of inputs some of which may require grad."""
+    if not torch.is_grad_enabled():
+        return outputs
+    inputs = [t for t in inputs if isinstance(t, torch.Tensor) and t.requires_grad]
+    return _NoBackward.apply(call, outputs, *inputs) if inputs else outputs
+
+
+def _given(t: torch.Tensor, name: str, *inputs) -> None:
+    """Refuses to write into ``t`` what autograd would have to follow."""
+    if torch.is_grad_enabled() and (t.requires_grad or any(i.requires_grad for i in inputs)):
+        raise ValueError(f"{name} where a tensor requires grad: there is no backward pass")
+
+
 class NormOutput(NamedTuple):
     q: torch.Tensor            # float8_e4m3fn, rows padded to 128 in memory
     scale: torch.Tensor        # float8_e8m0fnu, one for 128 values
@@ -165,6 +198,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *,
             raise ValueError("residual_out does not have x's shape and type")
         else:
             _on(residual_out, device, "residual_out")
+            _given(residual_out, "residual_out", x, residual)
         out = _rows(residual_out, "residual_out")
         out_ptr, out_stride = out.data_ptr(), out.stride(0)
     elif residual_out is not None:
@@ -185,6 +219,12 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *,
     if x.dim() != 2:
         q = q.view(x.shape)
         scale = scale.view(x.shape[:-1] + (blocks,))
+    if x.requires_grad or (residual is not None and residual.requires_grad):
+        outputs = (q, scale) if residual is None else (q, scale, residual_out)
+        q, scale, *rest = _untracked("rms_norm_fp8", outputs, x, weight, residual)
+        return NormOutput(q, scale, *(rest or [None]))
+    if weight.requires_grad:  # of which the sum knows nothing
+        q, scale = _untracked("rms_norm_fp8", (q, scale), weight)
     return NormOutput(q, scale, residual_out)
 
 
@@ -234,6 +274,7 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor,
             c = c[:, :n]
         out = c if a.dim() == 2 else c.view(a.shape[:-1] + (n,))
     else:
+        _given(out, "out", a, a_scale, w, w_scale)
         if out.shape != a.shape[:-1] + (n,):
             raise ValueError(f"out has shape {tuple(out.shape)}")
         _on(out, device, "out")
@@ -245,6 +286,8 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor,
         _raw_stream(device.index))
     if status:
         _fail(status, "tk_head_matmul")
+    if a.requires_grad or w.requires_grad or a_scale.requires_grad or w_scale.requires_grad:
+        out, = _untracked("matmul_fp8", (out,), a, a_scale, w, w_scale)
     return out
 
 
@@ -328,6 +371,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *,
         _raw_stream(device.index))
     if status:
         _fail(status, "tk_head_sample")
+    if logits.requires_grad or u.requires_grad or t_ptr or p_ptr or f_ptr:
+        ids, logprob = _untracked("sample", (ids, logprob), logits, u, temperature, top_p, min_p)
     return Sampled(ids, logprob)
 
 
@@ -337,7 +382,8 @@ def quantize_fp8(x: torch.Tensor, chunk: int = 16384
     values and, for each 128, the least power of two that holds their largest
     below e4m3's largest value. Done once when weights are loaded, in plain
     torch operations over ``chunk`` rows at a time. Rows are padded in memory
-    to a multiple of 128 with zeros."""
+    to a multiple of 128 with zeros. The result does not require grad, whether
+    or not x does."""
     if x.dim() != 2 or not x.is_floating_point():
         raise ValueError("rows of floats are wanted")
     n, k = x.shape
@@ -363,9 +409,9 @@ class OutputHead:
     vocabulary projection, next token.
 
     ``norm_weight``: ``[k]``; ``w``, ``w_scale``: the projection ``[n, k]`` in
-    8 bits (``quantize_fp8``). ``vocab``: the tokens that may be drawn, where
-    the projection's rows are padded beyond the tokenizer's ids (its
-    vocabulary with the added tokens)."""
+    8 bits (``quantize_fp8``); all three are held detached. ``vocab``: the
+    tokens that may be drawn, where the projection's rows are padded beyond the
+    tokenizer's ids (its vocabulary with the added tokens)."""
 
     def __init__(self, norm_weight: torch.Tensor, w: torch.Tensor,
                  w_scale: torch.Tensor, *, eps: float = 1e-6,
@@ -377,8 +423,8 @@ class OutputHead:
             raise ValueError(f"vocab {vocab} of {w.shape[0]} rows")
         if logits_dtype not in (torch.bfloat16, torch.float16):
             raise TypeError("logits come in bfloat16 or float16")
-        self.norm_weight = norm_weight
-        self.w, self.w_scale = _eight(w, w_scale, "w")
+        self.norm_weight = norm_weight.detach()
+        self.w, self.w_scale = _eight(w.detach(), w_scale.detach(), "w")
         if vocab is not None:
             self.w, self.w_scale = self.w[:vocab], self.w_scale[:vocab]
         self.eps = eps
