@@ -342,3 +342,24 @@ def test_an_output_head_holds_its_weights_detached(stand):
     got = out.next_ids(needs(torch.randn(2, 256)), torch.rand(2))
     with pytest.raises(NotImplementedError):
         got.logprob.sum().backward()
+
+
+def test_what_is_written_in_place_is_known_to_autograd(stand):
+    """A graph that saved a tensor notices that a call wrote over it."""
+    x, w, r = torch.randn(2, 256), torch.ones(256), torch.randn(2, 256)
+    a, b, out = eight(2, 256), eight(40, 256), torch.zeros(2, 40, dtype=torch.bfloat16)
+    read = [(t, t._version) for t in (x, w, *a, *b)]
+    factor = needs(torch.ones(2, 256))
+    saved = (factor * r).sum()
+    head.rms_norm_fp8(x, w, residual=r, residual_out=r)
+    with pytest.raises(RuntimeError, match="inplace"):
+        saved.backward()
+    saved = (needs(torch.ones(2, 40, dtype=torch.bfloat16)) * out).sum()
+    head.matmul_fp8(*a, *b, out=out)
+    with pytest.raises(RuntimeError, match="inplace"):
+        saved.backward()
+    # what is only read is not marked
+    assert all(t._version == version for t, version in read)
+    with torch.inference_mode():
+        kept = torch.randn(2, 256)
+        assert head.rms_norm_fp8(kept, w, residual=kept, residual_out=kept).residual is kept

@@ -31,6 +31,7 @@ from pathlib import Path
 from typing import NamedTuple
 
 import torch
+from torch.autograd.graph import increment_version as _written
 
 from ._build import HEAD_LIB
 from ._ffi import EngineError
@@ -186,6 +187,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *,
         raise TypeError(f"weight is {weight_kind}: {kind} or float32 is wanted")
     _on(weight, device, "weight")
     res_ptr = res_stride = out_ptr = out_stride = 0
+    given = residual_out is not None
     if residual is not None:
         if residual.shape != x.shape or residual.dtype != kind:
             raise ValueError("residual does not have x's shape and type")
@@ -214,6 +216,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *,
         _raw_stream(device.index))
     if status:
         _fail(status, "tk_head_norm")
+    if given:
+        _written(residual_out)
     if padded != k:
         q = q[:, :k]
     if x.dim() != 2:
@@ -268,7 +272,8 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor,
     _on(a_scale, device, "a_scale")
     _on(w, device, "w")
     _on(w_scale, device, "w_scale")
-    if out is None:
+    given = out is not None
+    if not given:
         c = a.new_empty((m, (n + 7) // 8 * 8), dtype=out_dtype)
         if n % 8:
             c = c[:, :n]
@@ -286,6 +291,8 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor,
         _raw_stream(device.index))
     if status:
         _fail(status, "tk_head_matmul")
+    if given:
+        _written(out)
     if a.requires_grad or w.requires_grad or a_scale.requires_grad or w_scale.requires_grad:
         out, = _untracked("matmul_fp8", (out,), a, a_scale, w, w_scale)
     return out
