@@ -28,6 +28,7 @@
 extern "C" {
 #endif
 
+/* what tk_head_abi_version returns; another with any change of a struct */
 #define TKH_ABI_VERSION 1
 #define TKH_OK 0
 #define TKH_E_INVALID_ARG (-1)
@@ -136,6 +137,11 @@ int tk_head_sample(const tkh_sample* args, void* stream);
 uint64_t tk_head_sample_workspace(int64_t rows, int64_t vocab, int32_t dtype);
 
 const char* tk_head_last_error(void);
+
+/* TKH_ABI_VERSION of the library, and the digest of the sources and flags
+ * that it was built from. */
+int tk_head_abi_version(void);
+const char* tk_head_sources(void);
 
 #ifdef __cplusplus
 }

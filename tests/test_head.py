@@ -363,3 +363,39 @@ def test_what_is_written_in_place_is_known_to_autograd(stand):
     with torch.inference_mode():
         kept = torch.randn(2, 256)
         assert head.rms_norm_fp8(kept, w, residual=kept, residual_out=kept).residual is kept
+
+
+def test_the_librarys_arguments_are_those_that_are_packed():
+    defined = int(re.search(r"#define\s+TKH_ABI_VERSION\s+(\d+)", HEADER.read_text()).group(1))
+    assert head.lib().tk_head_abi_version() == head.ABI_VERSION == defined
+    # csrc/head/head_api.cpp holds the structs to the same sizes
+    assert (head._NORM.size, head._MATMUL.size, head._SAMPLE.size) == (120, 112, 144)
+
+
+def test_a_library_of_other_arguments_is_refused(tmp_path):
+    import subprocess
+    names = [n for n in head.SYMBOLS if n != "tk_head_abi_version"]
+    for extra in ("", "int tk_head_abi_version(void) { return %d; }" % (head.ABI_VERSION + 1)):
+        src, so = tmp_path / "other.c", tmp_path / f"other{len(extra)}.so"
+        src.write_text("".join(f"int {n}(void) {{ return 0; }}\n" for n in names) + extra)
+        subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(so), str(src)], check=True)
+        with pytest.raises(RuntimeError, match="build it again"):
+            head.lib(so)
+
+
+def test_the_library_is_of_the_present_sources(monkeypatch, tmp_path):
+    from toktier_amd import _build
+    assert _build.verify_head() is None
+    here = tmp_path / "head"
+    here.mkdir()
+    for f in _build.HEAD_SRC.iterdir():
+        (here / f.name).write_bytes(f.read_bytes())
+    monkeypatch.setattr(_build, "HEAD_SRC", here)
+    assert _build.verify_head() is None
+    with open(here / "head_common.h", "a") as f:
+        f.write("// edited\n")
+    assert "sources" in _build.verify_head()
+    with pytest.warns(RuntimeWarning, match="sources"):
+        head.lib(_build.HEAD_LIB)
+    monkeypatch.setattr(_build, "HEAD_LIB", tmp_path / "none.so")
+    assert "missing" in _build.verify_head()

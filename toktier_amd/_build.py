@@ -9,6 +9,7 @@ offload architecture, the hipcc version and the exported ``tk_*`` symbols
 
 from __future__ import annotations
 
+import ctypes as C
 import hashlib
 import json
 import os
@@ -32,6 +33,7 @@ SOURCES = ["tk_device.hip", "tk_added.hip", "tk_engine.cpp"]
 # evidence and the counter summaries stay those of the encode path.
 HEAD_SRC = CSRC / "head"
 HEAD_LIB = LIBDIR / "libtoktier_head.so"
+HEAD_ABI_HEADER = ROOT / "include" / "toktier_head.h"
 HEAD_SOURCES = ["head_norm.hip", "head_matmul.hip", "head_sample.hip",
                 "head_api.cpp"]
 
@@ -123,10 +125,21 @@ def build(verbose: bool = False) -> Path:
     return LIB
 
 
+def head_digest() -> str:
+    """Digest of what ``libtoktier_head.so`` is built from: its sources, its
+    header and the flags. The library holds the one that it was built from."""
+    files = [f for f in sorted(HEAD_SRC.iterdir()) if f.suffix in (".hip", ".cpp", ".h")]
+    body = json.dumps({"sources": {f.name: hashlib.sha256(f.read_bytes()).hexdigest()
+                                   for f in (*files, HEAD_ABI_HEADER)},
+                       "flags": HIPCC_FLAGS}, sort_keys=True)
+    return hashlib.sha256(b"toktier-head-build\0" + body.encode()).hexdigest()
+
+
 def build_head(verbose: bool = False) -> Path:
     """Build ``libtoktier_head.so`` (one compiler per source, then a link)."""
     LIBDIR.mkdir(exist_ok=True)
     compile_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+    compile_flags.append(f'-DTKH_SOURCES="{head_digest()}"')
     objs, running = [], []
     for src in HEAD_SOURCES:
         obj = LIBDIR / f"{src}.{os.getpid()}.o"
@@ -173,6 +186,22 @@ def verify(manifest: dict | None = None) -> str | None:
     changed = sorted(k for k in set(now) | set(was) if now.get(k) != was.get(k))
     if changed:
         return "sources changed since the build: " + ", ".join(changed)
+    return None
+
+
+def verify_head(lib: Path | None = None) -> str | None:
+    """None when ``libtoktier_head.so`` is there and was built from the
+    present sources, or where no sources are; else what differs."""
+    lib = HEAD_LIB if lib is None else lib
+    if not lib.exists():
+        return "library missing"
+    if not HEAD_SRC.is_dir() or not HEAD_ABI_HEADER.exists():
+        return None
+    sources = getattr(C.CDLL(str(lib)), "tk_head_sources", None)
+    if sources is not None:
+        sources.restype = C.c_char_p
+    if sources is None or sources().decode() != head_digest():
+        return "sources or flags changed since the build"
     return None
 
 

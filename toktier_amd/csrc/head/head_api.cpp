@@ -53,4 +53,11 @@ DeviceScope::~DeviceScope() {
 
 }  // namespace tkh
 
+// callers pack these by position
+static_assert(TKH_ABI_VERSION == 1 && sizeof(tkh_norm) == 120 && sizeof(tkh_matmul) == 112 &&
+                  sizeof(tkh_sample) == 144,
+              "other arguments are another TKH_ABI_VERSION");
+
 extern "C" const char* tk_head_last_error(void) { return tkh::g_message; }
+extern "C" int tk_head_abi_version(void) { return TKH_ABI_VERSION; }
+extern "C" const char* tk_head_sources(void) { return TKH_SOURCES; }

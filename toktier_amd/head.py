@@ -27,13 +27,14 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
+import warnings
 from pathlib import Path
 from typing import NamedTuple
 
 import torch
 from torch.autograd.graph import increment_version as _written
 
-from ._build import HEAD_LIB
+from ._build import HEAD_LIB, verify_head
 from ._ffi import EngineError
 
 __all__ = ["rms_norm_fp8", "matmul_fp8", "sample", "quantize_fp8",
@@ -49,7 +50,11 @@ _INF = float("inf")
 
 #: every entry point include/toktier_head.h declares
 SYMBOLS = ("tk_head_norm", "tk_head_matmul", "tk_head_sample",
-           "tk_head_sample_workspace", "tk_head_last_error")
+           "tk_head_sample_workspace", "tk_head_last_error",
+           "tk_head_abi_version", "tk_head_sources")
+
+#: TKH_ABI_VERSION of the structs packed below
+ABI_VERSION = 1
 
 # The argument structs of include/toktier_head.h, packed in one step: a call
 # of a single token lasts a few microseconds, and so would filling a
@@ -62,7 +67,8 @@ _lib: C.CDLL | None = None
 
 
 def lib(path: Path | None = None) -> C.CDLL:
-    """Load the library (``RuntimeError`` if it was never built)."""
+    """Load the library (``RuntimeError`` if it was never built or takes other
+    arguments; a ``RuntimeWarning`` if its sources have changed since)."""
     global _lib
     if _lib is not None and path is None:
         return _lib
@@ -72,6 +78,14 @@ def lib(path: Path | None = None) -> C.CDLL:
             f"{p} is missing: build it with toktier_amd._build.build_head() "
             "(hipcc --offload-arch=gfx950); there is no CPU fallback")
     L = C.CDLL(str(p))
+    # an older library would read the packed arguments by other fields
+    version = L.tk_head_abi_version() if hasattr(L, "tk_head_abi_version") else 0
+    if version != ABI_VERSION:
+        raise RuntimeError(f"{p} takes arguments of version {version}, not {ABI_VERSION}: "
+                           "build it again with toktier_amd._build.build_head()")
+    stale = verify_head(p)
+    if stale:
+        warnings.warn(f"{p}: {stale}", RuntimeWarning, stacklevel=2)
     for name in ("tk_head_norm", "tk_head_matmul", "tk_head_sample"):
         f = getattr(L, name)
         f.restype = C.c_int
