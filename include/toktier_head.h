@@ -53,7 +53,8 @@ extern "C" {
  * 128; 2^22 rows to sample from, fewer of long ones (2^12 of the widest). */
 
 /* y = (x + residual) * rsqrt(mean((x + residual)^2) + eps) * weight in
- * 32 bits, then for each block of 128 the least power of two s with
+ * 32 bits (of h scaled by a power of two where its squares are beyond them:
+ * a finite row has a finite norm), then for each block of 128 the least power of two s with
  * amax <= 448 s (1 for a block of zeros), q = e4m3(y / s). Values that are
  * not finite become NaN and do not count for amax. residual_out (optional;
  * may be residual itself) receives x + residual in x's type. The pad of a

@@ -653,3 +653,24 @@ def test_inputs_that_require_grad_give_the_same_and_no_gradient():
     assert x.grad is None
     with pytest.raises(ValueError, match="residual_out"):
         head.rms_norm_fp8(x, w, residual=r, residual_out=r)
+
+
+@pytest.mark.parametrize("k", [1, 128, 1000, 5001, 40000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size,eps", [(1e19, 1e-6), (3e21, 1e-6), (5e30, 0.0), (3e38, 1e-6), (3e38, 3e38),
+                                      (1e-18, 0.0), (1e-25, 0.0), (1e-25, 1e-30), (1e-39, 0.0),
+                                      (1e-25, 1e-6), (1e-12, 5e-20)])
+def test_norm_of_rows_whose_squares_leave_32_bits(k, dtype, size, eps):
+    """Finite rows have finite norms: squares above 2^128 or below 2^-126."""
+    g = gen(k)
+    x = (size * (1 - 2 * torch.rand(4, k, generator=g, device="cuda", dtype=torch.float64))).to(DT[dtype])
+    x[1, k // 2:] *= 1e-3
+    x[2] = size
+    w = (1 + 0.2 * randn(g, k)).to(DT[dtype])
+    out = head.rms_norm_fp8(x, w, eps=eps)
+    # a row that the thousandth leaves at zero is 0 / 0 where eps is 0
+    none = (x == 0).all(-1) & (eps == 0)
+    assert bool(out.q[none].float().isnan().all())
+    for r in torch.nonzero(~none).flatten().tolist():
+        cut = slice(r, r + 1)
+        check_norm(x[cut], None, w, eps, out._replace(q=out.q[cut], scale=out.scale[cut]))

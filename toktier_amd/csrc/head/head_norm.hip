@@ -33,6 +33,16 @@ __device__ __forceinline__ float sum64(float v) {
     return v;
 }
 
+// The sum over a workgroup, in every lane; `part` is used once.
+__device__ __forceinline__ float block_sum(float (&part)[16], float v, int t, int threads) {
+    v = sum64(v);
+    if ((t & 63) == 0) part[t >> 6] = v;
+    __syncthreads();
+    float sum = 0.0f;
+    for (int i = 0; i < threads >> 6; ++i) sum += part[i];
+    return sum;
+}
+
 // The least e with amax <= 448 * 2^e (448 = 0.875 * 2^9), 0 for a block of
 // zeros, within what a scale byte holds.
 __device__ __forceinline__ int scale_exponent(float amax) {
@@ -47,7 +57,7 @@ template <typename T, typename W, int VPT>
 __global__ __launch_bounds__(1024) void k_norm(const tkh_norm p) {
     typedef typename Raw<T>::type R;
     typedef typename Raw<W>::type RW;
-    __shared__ float part[16];
+    __shared__ float part[2][16];
     const int64_t row = blockIdx.x;
     const int k = (int)p.k, t = threadIdx.x, threads = blockDim.x;
     const R* x = (const R*)p.x + row * p.x_stride;
@@ -93,12 +103,27 @@ __global__ __launch_bounds__(1024) void k_norm(const tkh_norm p) {
             }
         }
     }
-    sum = sum64(sum);
-    if ((t & 63) == 0) part[t >> 6] = sum;
-    __syncthreads();
-    sum = 0.0f;
-    for (int i = 0; i < threads >> 6; ++i) sum += part[i];
-    const float rstd = 1.0f / sqrtf(sum * (ldexpf(1.0f, log_k) / (float)k) + p.eps);
+    const float over_k = ldexpf(1.0f, log_k) / (float)k;
+    float mean = block_sum(part[0], sum, t, threads) * over_k, eps = p.eps;
+    // Where the mean or its sum with eps is infinite, or the mean may have lost
+    // squares to underflow and eps does not hide that, it is taken of h times a
+    // power of two, and eps with it: the largest such h is below 2^62, and the
+    // smallest, of 2^-149, has a square of 2^-106. An h that is infinite itself
+    // leaves the mean infinite.
+    if (mean + eps == INFINITY || (mean < 0x1p-95f && eps < 0x1p-64f)) {
+        const float scale = mean < 1.0f ? 0x1p96f : 0x1p-66f;
+        eps = eps * scale * scale;
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                h[i][j] *= scale;
+                sum += (h[i][j] * part_k) * h[i][j];
+            }
+        mean = block_sum(part[1], sum, t, threads) * over_k;
+    }
+    const float rstd = 1.0f / sqrtf(mean + eps);
 
     const RW* w = (const RW*)p.weight;
     uint8_t* q = (uint8_t*)p.q + row * p.q_stride;
