@@ -399,3 +399,17 @@ def test_the_library_is_of_the_present_sources(monkeypatch, tmp_path):
         head.lib(_build.HEAD_LIB)
     monkeypatch.setattr(_build, "HEAD_LIB", tmp_path / "none.so")
     assert "missing" in _build.verify_head()
+
+
+def test_settings_of_another_kind_are_type_errors(stand):
+    logits, u = torch.randn(2, 40), torch.rand(2)
+    for kw in (dict(top_k=5.0), dict(top_k="5"), dict(temperature="1"), dict(top_p=None), dict(min_p=[0.1])):
+        with pytest.raises(TypeError, match=next(iter(kw))):
+            head.sample(logits, u, **kw)
+    for eps in ("1e-6", None):
+        with pytest.raises(TypeError, match="eps"):
+            head.rms_norm_fp8(torch.randn(2, 40), torch.ones(40), eps=eps)
+    assert stand.names() == []
+    import numpy as np
+    head.sample(logits, u, top_k=np.int64(5), temperature=np.float32(0.5), top_p=1)
+    assert stand.calls[-1][1][16] == 5 and stand.calls[-1][1][15] == 0.5

@@ -26,6 +26,7 @@ pass that reaches them raises; what would have to be written into ``out`` or
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import struct
 import warnings
 from pathlib import Path
@@ -188,6 +189,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *,
     and ``scale`` have x's leading axes; q's rows are padded in memory to a
     multiple of 128 with zeros. Values that are not finite become NaN."""
     device = _gpu(x, "x")
+    if not hasattr(eps, "__float__"):
+        raise TypeError(f"eps is {eps!r}: a number is wanted")
     kind = x.dtype
     dtype = _DTYPES.get(kind)
     if dtype is None:
@@ -326,7 +329,13 @@ def _setting(v, rows: int, dtype: torch.dtype, device: torch.device, name: str,
             raise ValueError(f"{name} is a number or a dense {dtype} tensor of {rows}")
         _on(v, device, name)
         return v.data_ptr(), 0
-    if not low <= v <= high:
+    try:
+        fits = low <= v <= high
+        if dtype is torch.int32:
+            v = operator.index(v)
+    except TypeError:
+        raise TypeError(f"{name} is {v!r}: a number or a {dtype} tensor is wanted") from None
+    if not fits:
         raise ValueError(f"{name} is {v}: {low} to {high} is wanted")
     return 0, v
 
