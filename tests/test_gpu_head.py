@@ -674,3 +674,59 @@ def test_norm_of_rows_whose_squares_leave_32_bits(k, dtype, size, eps):
     for r in torch.nonzero(~none).flatten().tolist():
         cut = slice(r, r + 1)
         check_norm(x[cut], None, w, eps, out._replace(q=out.q[cut], scale=out.scale[cut]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norm_whose_output_is_infinite_is_nan_there(dtype):
+    """Infinite weights and products beyond 32 bits: NaN in their places, which
+    the scale of their block does not count."""
+    k = 512
+    x = torch.ones(2, k, device="cuda", dtype=DT[dtype])
+    w = torch.ones(k, device="cuda", dtype=DT[dtype])
+    w[3], w[130], w[131], w[300] = INF, -INF, math.nan, INF
+    out = head.rms_norm_fp8(x, w, eps=0.0)
+    got = wide(out.q, out.scale)
+    bad = torch.zeros(2, k, dtype=torch.bool, device="cuda")
+    bad[:, [3, 130, 131, 300]] = True
+    assert torch.equal(got.isnan(), bad)
+    assert bool((got[~bad] == 1).all())
+    assert out.scale.view(torch.uint8).tolist() == [[127 - 8] * 4] * 2  # 1 is 256 * 2^-8
+    # one value of a row of zeros is sqrt(k) = 22 after the norm
+    x = torch.zeros(2, k, device="cuda", dtype=DT[dtype])
+    x[:, 200] = 2.0
+    w = torch.ones(k, device="cuda", dtype=DT[dtype])
+    w[200] = torch.finfo(DT[dtype]).max
+    out = head.rms_norm_fp8(x, w)
+    got = wide(out.q, out.scale)
+    assert bool(got[:, 200].isnan().all()) and float(got.nan_to_num(0).abs().sum()) == 0
+
+
+@pytest.mark.parametrize("k", [257, 1000, 4096])
+def test_norm_writes_the_sum_into_a_strided_view(k):
+    g = gen(k)
+    x, r = randn(g, 7, k).bfloat16(), randn(g, 7, k).bfloat16()
+    w = (1 + 0.2 * randn(g, k)).bfloat16()
+    store = torch.full((7, k + 21), 5.0, device="cuda", dtype=torch.bfloat16)
+    view = store[:, 9:9 + k]
+    out = head.rms_norm_fp8(x, w, residual=r, residual_out=view)
+    assert out.residual is view
+    check_norm(x, r, w, 1e-6, out)
+    assert bool((store[:, :9] == 5).all()) and bool((store[:, 9 + k:] == 5).all())
+    view.copy_(r)
+    again = head.rms_norm_fp8(x, w, residual=view, residual_out=view)
+    assert torch.equal(again.residual, out.residual)
+    assert torch.equal(again.q.view(torch.uint8), out.q.view(torch.uint8))
+
+
+@pytest.mark.parametrize("rows,vocab,kind,settings", [
+    (40, 20011, "normal", dict(top_p=0.95)), (33, 20011, "normal", dict(top_p=0.99, temperature=1.5)),
+    (70, 9001, "normal", dict(top_p=0.97, min_p=0.01)), (300, 5003, "normal", dict(top_p=0.95)),
+    (70, 5003, "steps", dict(top_p=0.98, temperature=2.0)), (270, 5003, "flat", dict(top_p=0.9))])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_sample_more_wide_rows_than_a_turn_takes(rows, vocab, kind, settings, dtype):
+    """Sets of over 2,048 tokens in more rows than 32, or 256."""
+    x = rows_of(kind, rows, vocab, dtype, rows)
+    share = torch.softmax(x.double() / settings.get("temperature", 1.0), -1).sort(descending=True).values
+    kept = (share.cumsum(-1) - share < settings["top_p"]).sum(-1)
+    assert int((kept > 2048).sum()) > (256 if rows > 256 else 32) or "min_p" in settings
+    check_rows(x, torch.rand(rows, generator=gen(rows), device="cuda"), **settings)
