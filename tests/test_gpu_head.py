@@ -730,3 +730,15 @@ def test_sample_more_wide_rows_than_a_turn_takes(rows, vocab, kind, settings, dt
     kept = (share.cumsum(-1) - share < settings["top_p"]).sum(-1)
     assert int((kept > 2048).sum()) > (256 if rows > 256 else 32) or "min_p" in settings
     check_rows(x, torch.rand(rows, generator=gen(rows), device="cuda"), **settings)
+
+
+def test_a_refused_device_leaves_no_error_behind():
+    """A failed query's error would be raised by the next check of a launch,
+    torch's among them."""
+    p = 1 << 20  # an address that no call reads
+    lib = head.lib()
+    torch.zeros(1, device="cuda")
+    norm = [p, 0, p, p, p, 0, 4, 256, 256, 0, 256, 2, 0, 1e-6, 0, 0, 63]
+    assert lib.tk_head_norm(head._NORM.pack(*norm), None) == -3
+    assert lib.hipPeekAtLastError() == 0
+    assert float(torch.ones(3, device="cuda").sum()) == 3

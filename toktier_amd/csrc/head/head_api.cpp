@@ -18,6 +18,11 @@ int fail(int status, const char* fmt, ...) {
     return status;
 }
 
+int fail_hip(const char* what, hipError_t e) {
+    (void)hipGetLastError();  // taken back, so that no later check reports it
+    return fail(TKH_E_DEVICE, "%s: %s", what, hipGetErrorString(e));
+}
+
 // 0 unknown, 1 gfx950, 2 another architecture
 static std::atomic<int> g_arch[64];
 
@@ -27,8 +32,7 @@ static int check_arch(int device) {
     if (!known) {
         hipDeviceProp_t prop;
         hipError_t e = hipGetDeviceProperties(&prop, device);
-        if (e != hipSuccess)
-            return fail(TKH_E_DEVICE, "hipGetDeviceProperties: %s", hipGetErrorString(e));
+        if (e != hipSuccess) return fail_hip("hipGetDeviceProperties", e);
         known = strncmp(prop.gcnArchName, "gfx950", 6) == 0 ? 1 : 2;
         g_arch[device].store(known, std::memory_order_relaxed);
     }
@@ -44,7 +48,7 @@ DeviceScope::DeviceScope(int device) {
         e = hipSetDevice(device);
         if (e == hipSuccess) prev_ = now;
     }
-    if (e != hipSuccess) status_ = fail(TKH_E_DEVICE, "device %d: %s", device, hipGetErrorString(e));
+    if (e != hipSuccess) status_ = fail_hip("device", e);
 }
 
 DeviceScope::~DeviceScope() {

@@ -16,6 +16,9 @@ namespace tkh {
 // Records the message of tk_head_last_error and returns the status.
 int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 
+// The same for an error of the HIP runtime, which is left with none.
+int fail_hip(const char* what, hipError_t e);
+
 // Makes `device` current for a call and restores the caller's device after;
 // refuses a device that is not a gfx950.
 class DeviceScope {
@@ -36,8 +39,7 @@ int launch(const char* name, void (*kernel)(Params...), dim3 grid, dim3 block, s
         void* ptrs[] = {(void*)&p...};
         hipError_t e = hipLaunchKernel((const void*)kernel, grid, block, ptrs, lds,
                                        (hipStream_t)stream);
-        return e == hipSuccess ? TKH_OK
-                               : fail(TKH_E_DEVICE, "%s: %s", name, hipGetErrorString(e));
+        return e == hipSuccess ? TKH_OK : fail_hip(name, e);
     }(static_cast<Params>(args)...);
 }
 
