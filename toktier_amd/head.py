@@ -275,7 +275,9 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor,
     ``[..., ceil(k / 128)]`` of float8_e8m0fnu (or its bytes as uint8). Rows
     start at multiples of 16 bytes (``rms_norm_fp8`` and ``quantize_fp8`` give
     such rows for any k; of a single row only the address counts). The result
-    is ``[..., n]``, its rows at a multiple of 16 bytes in memory, or ``out``."""
+    is ``[..., n]``, its rows at a multiple of 16 bytes in memory, or ``out``.
+    How many rows a has decides the order of the sums: a row's values may
+    differ by a rounding from those that it has beside other rows."""
     device = _gpu(a, "a")
     dtype = _DTYPES.get(out_dtype if out is None else out.dtype)
     if dtype is None or dtype == TKH_F32:
@@ -351,8 +353,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *,
     or float16) from ``u``, one float32 in [0, 1) a row.
 
     A token weighs ``2**((x - max) * log2(e) / temperature)``, counted in whole
-    2**-40ths, so that a row's token does not depend on the batch it is in. In
-    the order of falling logits, equal ones by rising index, ``top_k`` keeps
+    2**-40ths, so that what a row's logits give does not depend on the batch
+    that they are in. In the order of falling logits, equal ones by rising index, ``top_k`` keeps
     that many (0: all); of them ``top_p`` keeps each that has less than its
     share of their weight before it; of those ``min_p`` keeps the ones of at
     least that share of the largest's weight. The token is the first by index
@@ -472,7 +474,9 @@ class OutputHead:
     def next_ids(self, x: torch.Tensor, u: torch.Tensor, *,
                  residual: torch.Tensor | None = None, **settings) -> Sampled:
         """One token for each of the hidden states ``[rows, k]``; settings as
-        in ``sample``."""
+        in ``sample``. The same call gives the same tokens; a row may get
+        another beside other rows, whose number decides how the product is
+        split and so the order of its 32-bit sums."""
         if x.dim() != 2:
             raise ValueError("hidden states have two axes")
         return sample(self.logits(x, residual=residual), u, **settings)
