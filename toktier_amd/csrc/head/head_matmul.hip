@@ -145,11 +145,12 @@ struct Rows {
 // 256 x 256 is the largest tile whose sums (128 registers a lane) and fragments
 // fit two waves a SIMD, and with 64 KB of operands for 2^23 products a step
 // comes closest to keeping the matrix units fed. 4096 x 4096 x 128256 takes
-// 1967 us, 2190 TF/s, the matrix units busy half of the clocks at 1.98 GHz: a
-// step's end waits for the next tiles, which come from L2 (operands are read
-// 6.3 times from beyond it). 200 x 4096 x 128256 takes 166 us, 3.2 TB/s of
-// weights: one tile of m, so that nothing is shared between workgroups. Where k
-// is short so is the whole: 24 x 1000 x 50257 14 us, 53 MB at 3.8 TB/s.
+// 1967 to 2091 us by the run, 2060 to 2190 TF/s, the matrix units busy half of
+// the clocks at 1.98 GHz: a step's end waits for the next tiles, which come from
+// L2 (operands are read 6.3 times from beyond it). 200 x 4096 x 128256 takes 169
+// us, 3.2 TB/s of weights: one tile of m, so that nothing is shared between
+// workgroups. Where k is short so is the whole: 24 x 1000 x 50257 14 us, 53 MB
+// at 3.8 TB/s.
 //
 // Tiles of one block of k lie in shared memory twice over, one being read while the
 // next arrives: a row takes 128 bytes, its 16-byte piece p at place p ^ (row
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void k_mm_tile(const tkh
         // the tiles, between the same waits as the others. Neighbouring waves
         // have the same rows and run on SIMDs of their own, so that the others
         // get the matrix units and the address unit for themselves: 777 x
-        // 2560 x 200019 478 us instead of 562, 300 x 4096 x 128256 240 / 276.
+        // 2560 x 200019 478 us instead of 562 (in turn), 300 x 4096 x 128256 240 / 276.
         bring_scales(0);
         if (whole) {
 #pragma unroll 1

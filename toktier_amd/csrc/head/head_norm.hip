@@ -8,9 +8,9 @@
 // registers through its sum, and the sum and q are written once. A workgroup
 // takes a row; a lane holds runs of 8 consecutive values, so that 16 lanes hold
 // a block of 128 and its maximum takes four exchanges within a row of lanes.
-// Measured: 16384 x 8192 bf16 with the residual 167 us, 940 MB moved (as many
-// as there are) at 5.6 TB/s; 1777 x 5001 floats 13.8 us alone and 12.7 us in a
-// row of calls, 44 MB at 3.5 TB/s; 1 x 4096 3.2 us.
+// Measured: 16384 x 8192 bf16 with the residual 168 us, 940 MB moved (as many
+// as there are) at 5.6 TB/s; 1777 x 5001 floats 14.1 us alone and 13.0 us in a
+// row of calls, 44 MB at 3.4 TB/s; 1 x 4096 3.3 us.
 #include "head_common.h"
 
 #include <math.h>

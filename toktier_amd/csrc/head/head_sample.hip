@@ -886,10 +886,10 @@ constexpr int kMostK = 1024, kFirst = 1024;
 // A workgroup a row. First turn: the rows with a top-k, and for the others
 // what k_masses needs. Second turn: those others. Bound by the length of the
 // steps that follow from each other, each ended by a barrier, not by what they
-// read or compute. One row of 151669 floats with top-k 50, 14.6 us of which:
+// read or compute. One row of 151669 floats with top-k 50, 15.0 us of which:
 // group keys and their largest 2, bins and the bin of the 50th 3, the tokens of
 // the groups that reach it 4.5, ranking them 5. The second turn over 256 rows of
-// 128256 bf16 with top-p 0.95 takes 25.5 us: 1 for the sums, 16 to gather
+// 128256 bf16 with top-p 0.95 takes 25.3 us: 1 for the sums, 16 to gather
 // the tokens of 1,024 groups or more, 6 to pick.
 template <typename T, bool Second> __global__ __launch_bounds__(kThreads) void k_pick(const tkh_sample p, const Work w) {
     __shared__ Shared s;

@@ -20,7 +20,7 @@ pass that reaches them raises; what would have to be written into ``out`` or
 
     head = OutputHead(norm_weight, *quantize_fp8(lm_head))
     out = head.next_ids(hidden, u, residual=residual, temperature=0.7, top_p=0.9)
-    out.ids        # int32 on the device: the ids that the tokenizer decodes
+    out.ids        # int32 on the device: rows of the projection, a tokenizer's ids
 """
 
 from __future__ import annotations
